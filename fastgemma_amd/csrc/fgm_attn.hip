@@ -353,7 +353,7 @@ __global__ __launch_bounds__(256) void attn_scores_kernel(const AttnArgs a) {
     const uint32_t base =
         slot < G.k_len ? (uint32_t)slot * (uint32_t)kvd + (uint32_t)(g * HD + 16 * (lane >> 4)) : FGM_OOB;
 #pragma unroll
-    for (int kk = 0; kk < KS; kk++) B[kk] = buf_load_b128(rk, base, 64 * kk);
+    for (int kk = 0; kk < KS; kk++) B[kk] = buf_load_b128(rk, base + 64u * kk, 0);
     kscale = buf_load_b32(rks, slot < G.k_len ? 4u * (uint32_t)slot : FGM_OOB, 0);
   };
   v4i B0[KS], B1[KS];
@@ -1288,7 +1288,7 @@ __global__ __launch_bounds__(64 * NW) void attn_fused_kernel(const AttnArgs a) {
     const uint32_t base = u < n ? (uint32_t)slot * (uint32_t)kvd + (uint32_t)(g * HD + 16 * q4) : FGM_OOB;
     kscale = buf_load_b32(rks, u < n ? 4u * (uint32_t)slot : FGM_OOB, 0);
 #pragma unroll
-    for (int kk = 0; kk < KS; kk++) B[kk] = buf_load_b128(rk, base, 64 * kk);
+    for (int kk = 0; kk < KS; kk++) B[kk] = buf_load_b128(rk, base + 64u * kk, 0);
   };
   v4i B0[KS], B1[KS];
   int ks0 = 0, ks1 = 0;
@@ -1328,7 +1328,7 @@ __global__ __launch_bounds__(64 * NW) void attn_fused_kernel(const AttnArgs a) {
     const int gi = (G.dom_slot(step) >> 2) + 4 * q4;
     const uint32_t at = ((uint32_t)gi * (uint32_t)kvd + (uint32_t)(g * HD + 64 * db + 4 * c16)) * 4u;
 #pragma unroll
-    for (int rr = 0; rr < 4; rr++) V[rr] = buf_load_b128(rv, at, (uint32_t)(rr * kvd * 4));
+    for (int rr = 0; rr < 4; rr++) V[rr] = buf_load_b128(rv, at + (uint32_t)(rr * kvd * 4), 0);
   };
   v4i V0[4], V1[4];
   if (sl < steps) loadv(V0, sl);

@@ -84,7 +84,9 @@ FGM_DEV int8_t quant_tail(float v) {
 
 // Raw buffer access (gfx9 buffer descriptor, no stride).  A lane whose byte
 // offset lies at or beyond `bytes` reads 0 without touching memory, which is
-// how the kernels mask rows and columns without branches.
+// how the kernels mask rows and columns without branches.  That check is on the
+// lane's own offset (voff and constants added to it) alone: what goes into soff
+// must not carry a lane that passes it past the end.
 constexpr int FGM_BUF_FLAGS = 0x00020000;  // gfx9 family descriptor word 3
 // An offset past the end of every buffer here, except a K or V cache of 2 GiB or
 // more (up to 4 GiB): attention uses nothing that a masked lane read from those.
