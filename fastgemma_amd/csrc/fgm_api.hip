@@ -1319,8 +1319,10 @@ int fgm_hip_attend_tree_dev(float* out, const float* q, const fgm_hip_tree_seq* 
   if ((rc = attn_scratch(a, max_span, scratch, scratch_bytes))) return rc;
   // a byte above each partial sum, in the place of the scores (256 cap bytes a pair)
   a.part_hi = (int8_t*)a.sc;
-  while (a.p3_chunks > 1 && a.p3_chunks * a.hd > 256 * a.cap)
-    a.p3_chunks = (a.tile_steps + ++a.p3_steps - 1) / a.p3_steps;
+  while (a.p3_chunks > 1 && a.p3_chunks * a.hd > 256 * a.cap) {
+    a.p3_steps++;
+    a.p3_chunks = (a.tile_steps + a.p3_steps - 1) / a.p3_steps;
+  }
   if ((rc = ensure_device())) return rc;
   hipError_t e = fgm_launch_attn_tree(a, (hipStream_t)stream);
   return e == hipSuccess ? FGM_HIP_OK : hip_fail(e, "tree attention launch");
