@@ -1052,6 +1052,11 @@ static int attn_check_heads(const AttnArgs& a) {
   return FGM_HIP_OK;
 }
 
+// K and V are addressed by 32-bit offsets.
+static bool cache_fits(int k_len, int kvh, int hd) {
+  return ((unsigned long long)k_len + 3) / 4 * 4 * (unsigned long long)kvh * hd < 1ull << 32;
+}
+
 // The grid of single rows or row tiles: rt, ntiles and tile_steps given.
 static void attn_grid(AttnArgs& a, bool tree = false) {
   // 64-slot steps per score workgroup: about 512 workgroups
@@ -1111,6 +1116,12 @@ static int attn_plan(AttnArgs& a, int* max_span) {
       steps_max = std::max(steps_max, sp.dom_steps);
       row_steps += sp.dom_steps;
       a.dup |= sp.lo0 < sp.hi1;
+    }
+    // a larger cache as one of the slots in use
+    if (s.nrows && !cache_fits(s.k_len, a.kvh, a.hd)) {
+      s.k_len = s.ring ? s.ring : s.pos0 + s.nrows;
+      if (!cache_fits(s.k_len, a.kvh, a.hd))
+        return fail(FGM_HIP_EINVAL, "attend: sequence %d: %d slots in use, 4 GiB or more", i, s.k_len);
     }
   }
   a.m = m;
@@ -1181,11 +1192,6 @@ static int attn_run(AttnArgs& a, void* scratch, size_t scratch_bytes, hipStream_
     return fail(FGM_HIP_EINVAL, "attend_mass: a slot domain of %d steps fills the scratch's %d", a.tile_steps, a.cap);
   hipError_t e = mass ? fgm_launch_attn_mass(a, *mass, st) : fgm_launch_attn(a, st);
   return e == hipSuccess ? FGM_HIP_OK : hip_fail(e, "attention launch");
-}
-
-// K and V are addressed by 32-bit offsets.
-static bool cache_fits(int k_len, int kvh, int hd) {
-  return ((unsigned long long)k_len + 3) / 4 * 4 * (unsigned long long)kvh * hd < 1ull << 32;
 }
 
 // attn_plan for drafted trees: a sequence's rows share one domain.
