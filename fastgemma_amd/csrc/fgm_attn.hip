@@ -1612,11 +1612,19 @@ hipError_t launch_softmax(const AttnArgs& a, hipStream_t st) {
     if (quads <= 2 * 512) return launch_softmax<MODE, 2, 512>(a, st);
     if (quads <= 3 * 512) return launch_softmax<MODE, 3, 512>(a, st);
     if (quads <= 4 * 512) return launch_softmax<MODE, 4, 512>(a, st);
-    // LATE: room for twice the workgroups (1024 pairs x 8208 slots 33.5 -> 27.4
-    // us, 512 x 16000 31.3 -> 24.2; with the registers of NQ <= 4 at 512 threads
-    // or the LDS of NQ > 5 at 1024 they have it either way or not at all)
+    // LATE: 64 registers, so that the LDS of up to 8960 positions has four workgroups
+    // of 512 a CU instead of three, that of 12289 to 19200 two of 1024 instead of
+    // one.  Measured both ways at 15 lengths, whole calls of 264, 512 and 1024
+    // pairs: attend, trees and weights of 12289 to 19200 positions 6 to 18 % faster
+    // (1024 pairs at 16000: attend 120.7 -> 102.5 us); five groups a thread from 4 %
+    // faster (1024 pairs at 8300: trees 71.8 -> 69.1) to 3 % slower (264 at 8300:
+    // attend 37.0 -> 38.2), 19201 and more from 3 % faster to 4 % slower (weights).
+    // Six groups have three workgroups either way, and their spills cost 1 to 7 %,
+    // weights 10 to 18 % (512 pairs at 10300, attend 49.5 -> 52.3 us): not LATE.
+    // With the registers of NQ <= 4 at 512 threads or the LDS of NQ > 5 at 1024 there
+    // is no room to win.
     if (quads <= 5 * 512) return launch_softmax<MODE, 5, 512, true>(a, st);
-    if (quads <= 6 * 512) return launch_softmax<MODE, 6, 512, true>(a, st);
+    if (quads <= 6 * 512) return launch_softmax<MODE, 6, 512>(a, st);
     if (quads <= 4 * 1024) return launch_softmax<MODE, 4, 1024, true>(a, st);
     if (quads <= 5 * 1024) return launch_softmax<MODE, 5, 1024, true>(a, st);
   }
