@@ -239,8 +239,12 @@ int fgm_hip_kv_store_dev(const float *k, const float *v, int m, int row_len, int
 /* ------------------------------------- drafted trees and bounded caches
  * No counterpart in the reference.  All of it is asynchronous on `stream`,
  * allocates nothing, synchronises nothing and can be captured in a graph; what
- * is in device memory (masks, index lists, weights) may change from replay to
- * replay.  Results depend on the inputs alone, not on the launch.
+ * is in device memory (masks, index lists, weights, queries, caches) may change
+ * from replay to replay, what the descriptors hold by value (pos, rows, n, count,
+ * cap, ring) and the window are the captured call's.  The same call on the same
+ * inputs gives the same bytes.  What a sequence is batched with changes neither
+ * out nor keep nor a moved byte; its accumulated weights (mass) it may change by
+ * their float32 rounding.
  *
  * Attention of drafted trees.  The `rows` rows of sequence i are the nodes of a
  * tree (at most 64) whose K and V have been appended at positions pos, pos + 1,
@@ -253,9 +257,11 @@ int fgm_hip_kv_store_dev(const float *k, const float *v, int m, int row_len, int
  * function gives for a linear cache that holds the line (whose sums it takes modulo
  * 2^32; here they have 64 bits), and no slot of a ring counts twice.
  * ring: at least window + rows (or pos + rows where that is less).  Limits as
- * fgm_hip_attend_dev's (caches of 4 GiB are refused here); `scratch` likewise, of fgm_hip_attend_scratch_bytes(total
- * rows, ..., max_span) where max_span bounds every ring size and every
- * min(pos, window) + rows (window 0: pos + rows). */
+ * fgm_hip_attend_dev's (caches of 4 GiB are refused here, whatever is in use);
+ * `scratch` likewise, of fgm_hip_attend_scratch_bytes(total rows, ..., max_span)
+ * where max_span bounds every ring size and every min(pos, window) + rows (window
+ * 0: pos + rows).  No weights are added up: slots that a committed path brings into
+ * use have the mass that the caller gives them. */
 typedef struct fgm_hip_tree_seq {
   const int8_t *kc;
   const float *ks;
@@ -277,8 +283,9 @@ int fgm_hip_attend_tree_dev(float *out, const float *q, const fgm_hip_tree_seq *
  * [pos + rows] or NULL (not wanted):
  *   mass[i][s] = decay * mass[i][s] + sum over rows and heads of the softmax weight of s
  * where the first term is 0 for s >= pos (new slots) and for decay = 0.  Slots
- * from pos + rows on are not touched.  Linear caches only (ring = 0); decay
- * finite and not negative; no two sequences with the same mass. */
+ * from pos + rows on, and all of a sequence without rows, are not touched.  Linear
+ * caches only (ring = 0); decay finite and not negative; no two sequences with the
+ * same mass. */
 int fgm_hip_attend_mass_dev(float *out, const float *q, const fgm_hip_attn_seq *seqs,
                             float *const *mass, int nseq, int n_heads, int kv_heads, int head_dim,
                             int window, float decay, void *scratch, size_t scratch_bytes,

@@ -198,3 +198,39 @@ def test_mass_paths(name):
     assert np.all(np.abs(got[:end] - w.sum((0, 1)) - first) <= off)
     assert np.array_equal(got[end:].view(np.uint32), had[end:].view(np.uint32))
     assert kernel in launches(run), launches(run)
+
+
+# the other sequence of the batch: what it makes of the call
+BESIDE = {"long_rows": (3000, 2900, 2), "tiles": (5200, 5100, 64), "short": (90, 70, 3)}
+
+
+@pytest.mark.parametrize("beside", BESIDE)
+@pytest.mark.parametrize("pos,rows", [(400, 1), (900, 20), (2301, 40)])
+def test_alone_and_in_a_batch(pos, rows, beside):
+    """out's bytes do not depend on what a sequence is batched with; its weights are the
+    same for the same call, and else differ by their rounding alone."""
+    nh, kvh, hd = 8, 1, 64
+    rng = np.random.default_rng(pos)
+    cap2, pos2, rows2 = BESIDE[beside]
+    a, b = U.Cache(rng, pos + rows, hd), U.Cache(rng, cap2, hd)
+    q = queries(rng, rows + rows2, nh, hd)
+    t = H.torch()
+    da, db, dq = dev_cache(a), dev_cache(b), H.dev(q)
+    ma, mb = (words(K.tree_mask(U.random_tree(rng, n))) for n in (rows, rows2))
+    one, two = t.zeros((rows, nh, hd), device="cuda"), t.zeros((rows + rows2, nh, hd), device="cuda")
+    K.attend_tree(one, dq[:rows], [(*da, a.cap, 0, pos, ma)], nh, kvh, hd)
+    K.attend_tree(two, dq, [(*da, a.cap, 0, pos, ma), (*db, cap2, 0, pos2, mb)], nh, kvh, hd)
+    assert np.array_equal(H.host(one).view(np.uint32), H.host(two)[:rows].view(np.uint32))
+    alone = t.zeros(a.cap, device="cuda")
+    K.attend_mass(one, dq[:rows], [(*da, a.cap, 0, pos, rows, alone)], nh, kvh, hd)
+    batch = []
+    for _ in range(2):
+        m, m2 = t.zeros(a.cap, device="cuda"), t.zeros(cap2, device="cuda")
+        K.attend_mass(two, dq, [(*da, a.cap, 0, pos, rows, m), (*db, cap2, 0, pos2, rows2, m2)], nh, kvh, hd)
+        batch.append(H.host(m))
+    assert np.array_equal(H.host(one).view(np.uint32), H.host(two)[:rows].view(np.uint32))
+    assert np.array_equal(batch[0].view(np.uint32), batch[1].view(np.uint32))
+    w = weights64(q[:rows], a, pos, 0, nh, kvh)
+    off = weights_off(q[:rows], a, w, nh)
+    for got in (H.host(alone), batch[0]):
+        assert np.all(np.abs(got - w.sum((0, 1))) <= off)
