@@ -152,9 +152,7 @@ def prepare(case, seed):
         st["lens"] = _lens(g, c["ctx"], s)
         st["n"] = torch.tensor(st["lens"], device=DEV)
         st["keep"] = torch.empty(s, c["budget"], dtype=torch.int32, device=DEV)
-        if own:
-            from fastgemma_amd import kernels as K
-            st["descs"] = K.select_seqs([(st["keep"][i], st["mass"][i], n) for i, n in enumerate(st["lens"])])
+        st["seqs"] = [(st["keep"][i], st["mass"][i], n) for i, n in enumerate(st["lens"])]
         return st
     if c["kind"] == "move":
         slots = c["ctx"]
@@ -169,13 +167,11 @@ def prepare(case, seed):
             n = min(c["count"], span) if i == 0 else g.r.randint(1, min(c["count"], span) + 1)
             idx[i, :n] = _path(g, span, n)
         st["index"], st["first"] = torch.from_numpy(idx).to(DEV), torch.tensor(st["pos"], device=DEV)
-        if own:
-            from fastgemma_amd import kernels as K
-            ca = st["cache"]
-            st["descs"] = K.kv_moves([{
-                "src": (ca["kc"][i], ca["ks"][i], ca["vt"][i], ca["vs"][i], ca["mass"][i] if c["mass"] else None),
-                "cap": slots, "ring": slots if c["ring"] else 0, "pos": st["pos"][i], "index": st["index"][i]}
-                for i in range(s)], c["row"])
+        ca = st["cache"]
+        st["moves"] = [{
+            "src": (ca["kc"][i], ca["ks"][i], ca["vt"][i], ca["vs"][i], ca["mass"][i] if c["mass"] else None),
+            "cap": slots, "ring": slots if c["ring"] else 0, "pos": st["pos"][i], "index": st["index"][i]}
+            for i in range(s)]
         return st
     rows = c["nodes"] if c["kind"] == "tree" else c["rows"]
     nh, kvh, hd = c["nh"], c["kvh"], c["hd"]
@@ -193,15 +189,15 @@ def prepare(case, seed):
         # what the rows before these have given each slot, a few rows' worth in all
         st["mass"] = torch.exp(1.5 * g.normal(s, slots)) * (nh / c["ctx"])
     st["first"] = torch.tensor(st["pos"], device=DEV)
+    per = [(ca["kc"][i], ca["ks"][i], ca["vt"][i], ca["vs"][i], slots, slots if ring else 0, st["pos"][i])
+           for i in range(s)]
+    if c["kind"] == "tree":
+        st["seqs"] = [p + (st["mask"][i],) for i, p in enumerate(per)]
+    else:
+        st["seqs"] = [p + (rows, st["mass"][i]) for i, p in enumerate(per)]
     if own:
         from fastgemma_amd import kernels as K
-        per = [(ca["kc"][i], ca["ks"][i], ca["vt"][i], ca["vs"][i], slots, slots if ring else 0, st["pos"][i])
-               for i in range(s)]
-        if c["kind"] == "tree":
-            st["descs"] = K.tree_seqs([p + (st["mask"][i],) for i, p in enumerate(per)], c["window"])
-        else:
-            st["descs"] = K.mass_seqs([p + (rows, st["mass"][i]) for i, p in enumerate(per)])
-        nb = K.attend_scratch_bytes(s * rows, nh, kvh, hd, st["descs"].span)
+        nb = K.attend_scratch_bytes(s * rows, nh, kvh, hd, slots)
         st["scratch"] = torch.empty(nb + 256, dtype=torch.uint8, device=DEV)
     return st
 
@@ -299,12 +295,14 @@ def _move(ca, index, first, ring):
 
 
 # --------------------------------------------------------------------- run
+# Lengths and positions change from one decode step to the next, and the library's
+# descriptors hold them: a user's program makes those for each call, and so does run.
 def run(st):
     c = st["case"]
     if c["kind"] == "select":
         if own:
             from fastgemma_amd import kernels as K
-            K.kv_select(st["descs"], c["budget"], c["sink"], c["recent"])
+            K.kv_select(st["seqs"], c["budget"], c["sink"], c["recent"])
         else:
             st["keep"] = _select(st["mass"], st["n"], c["budget"], c["sink"], c["recent"])
         return {"keep": st["keep"]}
@@ -312,7 +310,7 @@ def run(st):
     if c["kind"] == "move":
         if own:
             from fastgemma_amd import kernels as K
-            K.kv_move(st["descs"])
+            K.kv_move(st["moves"], c["row"])
         else:
             _move(ca, st["index"], st["first"], c["ctx"] if c["ring"] else 0)
         # moved bytes are whole numbers that have to be equal
@@ -322,14 +320,14 @@ def run(st):
     if c["kind"] == "tree":
         if own:
             from fastgemma_amd import kernels as K
-            K.attend_tree(st["out"], st["q"], st["descs"], nh, kvh, hd, c["window"], st["scratch"])
+            K.attend_tree(st["out"], st["q"], st["seqs"], nh, kvh, hd, c["window"], st["scratch"])
         else:
             live = _tree_live(st["first"], st["mask"], slots, slots if c["ring"] else 0, c["window"])
             st["out"] = _attention(st["q"], ca, live, kvh)[0]
         return {"out": st["out"]}
     if own:
         from fastgemma_amd import kernels as K
-        K.attend_mass(st["out"], st["q"], st["descs"], nh, kvh, hd, decay=1.0, scratch=st["scratch"])
+        K.attend_mass(st["out"], st["q"], st["seqs"], nh, kvh, hd, decay=1.0, scratch=st["scratch"])
     else:
         st["out"], p = _attention(st["q"], ca, _row_live(st["first"], c["rows"], slots), kvh)
         st["mass"] = _add_mass(st["mass"], p, st["first"], c["rows"])
