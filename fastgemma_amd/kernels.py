@@ -544,13 +544,16 @@ def kv_store(k, v, m: int, row_len: int, kc, ks, vt, vs, cap: int, pos: int,
 
 
 # ------------------------------------- drafted trees and bounded caches
-# Device API only, no counterpart in the reference.  A serving loop calls these
-# with the same caches again and again, so the descriptors of a call are made
-# apart (tree_seqs, mass_seqs, select_seqs, kv_moves: checks and addresses) and
-# may be kept; each call also takes the plain list and makes them itself.
+# Device API only, no counterpart in the reference.  Each call takes a plain list
+# of its sequences and makes descriptors of it (checks and addresses, 2 to 4 us of
+# host time a sequence), or takes descriptors made apart (tree_seqs, mass_seqs,
+# select_seqs, kv_moves).  They hold positions, lengths and node counts as they were
+# when made: they serve the calls of one step, or a capture, and the next step,
+# whose positions are others, makes its own.
 class CacheDescs:
     """Descriptors of one call over several caches, kept with the tensors that
-    they point into.  `span`: what attend_scratch_bytes takes for them."""
+    they point into.  Positions and lengths are copied when they are made.
+    `span`: what attend_scratch_bytes takes for them."""
 
     __slots__ = ("kind", "arr", "count", "rows", "span", "row", "keep_len", "window", "mass", "device", "refs")
 
