@@ -1211,7 +1211,8 @@ static int tree_plan(AttnArgs& a, int* max_span) {
       return fail(FGM_HIP_EINVAL, "attend_tree: sequence %d has %d rows (at most %d)", i, s.nrows, FGM_TREE_MAX_ROWS);
     if (s.nrows && (!s.kc || !s.ks || !s.vc || !s.vs || !s.mask))
       return fail(FGM_HIP_EINVAL, "attend_tree: sequence %d has a NULL cache or mask pointer", i);
-    if ((uintptr_t)s.mask & 7) return fail(FGM_HIP_EINVAL, "attend_tree: sequence %d: mask is not aligned to 8 bytes", i);
+    if ((uintptr_t)s.mask & 7)
+      return fail(FGM_HIP_EINVAL, "attend_tree: sequence %d: mask is not aligned to 8 bytes", i);
     if (s.k_len <= 0 || s.ring < 0 || s.ring > s.k_len || s.pos0 < 0)
       return fail(FGM_HIP_EINVAL, "attend_tree: sequence %d: k_len=%d ring=%d pos=%d", i, s.k_len, s.ring, s.pos0);
     if (s.nrows && !cache_fits(s.k_len, a.kvh, a.hd))
@@ -1294,7 +1295,8 @@ int fgm_hip_attend_mass_dev(float* out, const float* q, const fgm_hip_attn_seq* 
     for (int j = 0; j < i; j++)
       if (w.mass[i] && w.mass[i] == w.mass[j])
         return fail(FGM_HIP_EINVAL, "attend_mass: sequences %d and %d share their weights", j, i);
-    if (w.mass[i]) w.max_slots = std::max<long long>(w.max_slots, std::min<long long>((long long)s.pos + s.rows, INT_MAX));
+    if (w.mass[i])
+      w.max_slots = std::max<long long>(w.max_slots, std::min<long long>((long long)s.pos + s.rows, INT_MAX));
   }
   for (int i = 0; i < nseq; i++)
     if (seqs[i].rows > 0 && seqs[i].k_len > 0 && kv_heads > 0 && head_dim > 0 &&
@@ -1384,7 +1386,8 @@ int fgm_hip_kv_move_dev(const fgm_hip_kv_move_desc* d, int count, int row_len, v
     if (x.count && !x.index) return fail(FGM_HIP_EINVAL, "kv_move[%d]: index is NULL", i);
     for (const fgm_hip_kv_cache* c : {&x.src, &x.dst}) {
       if (!c->kc || !c->ks || !c->vt || !c->vs) return fail(FGM_HIP_EINVAL, "kv_move[%d]: NULL buffer", i);
-      if (c->cap <= 0 || c->cap > FGM_CACHE_MAX || c->ring < 0 || c->ring > c->cap || c->pos < 0 || (!c->ring && c->pos > c->cap))
+      if (c->cap <= 0 || c->cap > FGM_CACHE_MAX || c->ring < 0 || c->ring > c->cap || c->pos < 0 ||
+          (!c->ring && c->pos > c->cap))
         return fail(FGM_HIP_EINVAL, "kv_move[%d]: cap=%d ring=%d pos=%d", i, c->cap, c->ring, c->pos);
     }
     if (!x.src.mass != !x.dst.mass) return fail(FGM_HIP_EINVAL, "kv_move[%d]: mass on one side only", i);

@@ -1126,7 +1126,8 @@ __global__ __launch_bounds__(256 * NG * KG, 2) void attn_pv_tile_kernel(const At
       } else {
         const size_t at = (row * a.p3_chunks + bz) * a.hd + d0 + 4 * c32;
         *(v4i*)(a.part + at) = v4i{(int)x[0], (int)x[1], (int)x[2], (int)x[3]};
-        *(uint32_t*)(a.part_hi + at) = pack4_i8((int)(x[0] >> 32), (int)(x[1] >> 32), (int)(x[2] >> 32), (int)(x[3] >> 32));
+        *(uint32_t*)(a.part_hi + at) =
+            pack4_i8((int)(x[0] >> 32), (int)(x[1] >> 32), (int)(x[2] >> 32), (int)(x[3] >> 32));
       }
       continue;
     }
@@ -1471,7 +1472,8 @@ __global__ __launch_bounds__(64 * NW) void attn_fused_kernel(const AttnArgs a) {
 #pragma unroll
   for (int i = 0; i < 4; i++) {
     const int row = 4 * q4 + i;
-    if (row < 3 * hpw) *(v4i*)(red + ((size_t)w * 3 * hpw + row) * 64 + 4 * c16) = v4i{D0[0][i], D0[1][i], D0[2][i], D0[3][i]};
+    if (row < 3 * hpw)
+      *(v4i*)(red + ((size_t)w * 3 * hpw + row) * 64 + 4 * c16) = v4i{D0[0][i], D0[1][i], D0[2][i], D0[3][i]};
     if (row + 16 < 3 * hpw)
       *(v4i*)(red + ((size_t)w * 3 * hpw + row + 16) * 64 + 4 * c16) = v4i{D1[0][i], D1[1][i], D1[2][i], D1[3][i]};
   }
@@ -1641,8 +1643,9 @@ hipError_t launch_softmax(const AttnArgs& a, hipStream_t st) {
 // ------------------------------------------------------- weights by slot
 // grid (64-slot blocks, sequences), T threads: the (row, head) pairs of a tile
 // (of a row, after the single launch, which leaves weights in the row's range
-// only; SUMS: exponentials, the reciprocal of their sum behind the row) are dealt to the T / 16 groups of 16 threads, four slots a thread, and
-// the groups' sums added in order: the order depends on the shapes alone.
+// only; SUMS: exponentials, the reciprocal of their sum behind the row) are dealt
+// to the T / 16 groups of 16 threads, four slots a thread, and the groups' sums
+// added in order: the order depends on the shapes of the call alone.
 // Bound by the read of the weights: 512 pairs x 16000 slots (33 MB) 7.5 us, 4.4
 // TB/s (16.9 us with 16 groups and a range check at each weight); 8 heads of one
 // row 3.0 us, a launch.
@@ -1704,7 +1707,8 @@ hipError_t launch_attn(const AttnArgs& a, hipStream_t st, bool* single = nullptr
   f.hpw = std::min(f.hpw, grp);
   const int nw = fused_waves(f);
   const size_t flds = fused_lds(nw, a.hd, f.hpw, a.max_n, a.max_steps);
-  const bool one = a.max_n <= fused_max_n(MODE, a.hd, a.m * a.nh) && grp <= FUSED_MAX_GRP && !(fz && fz[0] == '0') && flds <= 160 * 1024;
+  const bool one = a.max_n <= fused_max_n(MODE, a.hd, a.m * a.nh) && grp <= FUSED_MAX_GRP &&
+                   !(fz && fz[0] == '0') && flds <= 160 * 1024;
   if (single) *single = one;
   if (one)
     return with_ks(a.hd, [&](auto ks) {
@@ -1720,13 +1724,14 @@ hipError_t launch_attn(const AttnArgs& a, hipStream_t st, bool* single = nullptr
                        a.hd);
     if ((e = hipGetLastError()) != hipSuccess) return e;
     e = with_ks(a.hd, [&](auto ks) {
-      hipLaunchKernelGGL((attn_scores_tile_kernel<decltype(ks)::value, TREE>), dim3(chunks, a.ntiles * a.kvh), dim3(256), 0, st,
-                         a);
+      hipLaunchKernelGGL((attn_scores_tile_kernel<decltype(ks)::value, TREE>), dim3(chunks, a.ntiles * a.kvh),
+                         dim3(256), 0, st, a);
       return hipGetLastError();
     });
   } else {
     e = with_ks(a.hd, [&](auto ks) {
-      hipLaunchKernelGGL((attn_scores_kernel<decltype(ks)::value, TREE>), dim3(chunks, a.m * a.kvh), dim3(256), 0, st, a);
+      hipLaunchKernelGGL((attn_scores_kernel<decltype(ks)::value, TREE>), dim3(chunks, a.m * a.kvh), dim3(256), 0, st,
+                         a);
       return hipGetLastError();
     });
   }

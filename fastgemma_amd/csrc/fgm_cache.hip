@@ -287,7 +287,8 @@ hipError_t fgm_launch_move(const MoveBatch& b, bool in_place, hipStream_t st) {
   if (b.count <= 0 || b.row <= 0 || b.max_count <= 0) return hipSuccess;
   bool vec = b.row % 16 == 0;
   for (int i = 0; i < b.count; i++)
-    vec = vec && (((uintptr_t)b.p[i].kc | (uintptr_t)b.p[i].vt | (uintptr_t)b.p[i].kc_to | (uintptr_t)b.p[i].vt_to) & 15) == 0;
+    vec = vec && (((uintptr_t)b.p[i].kc | (uintptr_t)b.p[i].vt | (uintptr_t)b.p[i].kc_to |
+                   (uintptr_t)b.p[i].vt_to) & 15) == 0;
   const int slices = (b.row + KS - 1) / KS + (b.row + VS - 1) / VS + 1;
   auto launch = [&](auto t, auto in, auto v) {
     constexpr int T = decltype(t)::value;

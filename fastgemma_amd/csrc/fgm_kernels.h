@@ -220,9 +220,10 @@ __host__ __device__ inline int tree_start(int pos0, int window) {
 hipError_t fgm_launch_attn_tree(const AttnArgs& a, hipStream_t st);
 
 // Attention that also adds up the softmax weight of every slot (linear caches
-// only): the weights of each (row, head), or its exponentials and their sum, are
-// left in the place of its scores, then mass[i][s] = decay * mass[i][s] (s < pos0, else 0) + their sum over the
-// rows and heads of sequence i, for the slots s < pos0 + nrows.
+// only): the weights of each (row, head), or its exponentials and one over their
+// sum, are left in the place of its scores, then mass[i][s] = decay * mass[i][s]
+// (s < pos0, else 0) + the weights' sum over the rows and heads of sequence i, for
+// the slots s < pos0 + nrows.
 struct MassArgs {
   float* mass[FGM_ATTN_MAX_SEQ];  // NULL: not wanted for that sequence
   float decay;

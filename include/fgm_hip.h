@@ -284,8 +284,8 @@ int fgm_hip_attend_tree_dev(float *out, const float *q, const fgm_hip_tree_seq *
  *   mass[i][s] = decay * mass[i][s] + sum over rows and heads of the softmax weight of s
  * where the first term is 0 for s >= pos (new slots) and for decay = 0.  Slots
  * from pos + rows on, and all of a sequence without rows, are not touched.  Linear
- * caches only (ring = 0); decay finite and not negative; no two sequences with the
- * same mass. */
+ * caches under 4 GiB only (ring = 0); decay finite and not negative; no two
+ * sequences with the same mass. */
 int fgm_hip_attend_mass_dev(float *out, const float *q, const fgm_hip_attn_seq *seqs,
                             float *const *mass, int nseq, int n_heads, int kv_heads, int head_dim,
                             int window, float decay, void *scratch, size_t scratch_bytes,
